@@ -301,7 +301,8 @@ int vcsrmc_mx_dequantise(const void *codes, const void *scales, long long rows, 
 
 /* Root-mean-square norm with the residual's addition, into MX:
  *   h = x + residual,  MX of  h / sqrt(mean(h^2) + eps) * weight,
- * row by row, h in 32 bits; residual_out = h rounded to `type`.  residual and residual_out may be
+ * row by row, h in 32 bits; residual_out = h rounded to `type`.  A normalised value that rounds past
+ * the largest 32-bit number is an infinity, so its block is NaN.  residual and residual_out may be
  * NULL (no addition; no copy), and residual_out may be x or residual themselves, with the same
  * stride.  weight holds cols values of weight_type, which is `type` or VCSRMC_TYPE_F32. */
 int vcsrmc_rms_norm_mx(const void *x, const void *residual, const void *weight, int type,

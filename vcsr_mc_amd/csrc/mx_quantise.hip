@@ -125,11 +125,13 @@ __device__ __forceinline__ void load_h(const RmsNormArgs& a, long long row, int 
 
 // v in 32 bits such that rounding the result to fewer bits is rounding v: the nearest number, or,
 // where that is even and not v, its neighbour on v's side.  (Boundaries of shorter formats are even.)
+// What rounds past the largest 32-bit number stays an infinity, which makes its block NaN: its
+// neighbour would be a finite value far below v.
 __device__ __forceinline__ float round_to_odd(double v) {
     const float f = (float)v;
-    const double d = v - (double)f;  // 0 or NaN for infinities and NaN
+    const double d = v - (double)f;  // not finite where f is not
     const unsigned u = __float_as_uint(f);
-    if ((u & 1) || !(d < 0 || d > 0)) return f;
+    if ((u & 1) || !(fabs(d) > 0 && fabs(d) < HUGE_VAL)) return f;
     return __uint_as_float((d > 0) == !(u >> 31) ? u + 1 : u - 1);
 }
 
