@@ -4,7 +4,7 @@ import pytest
 
 import mx_plain as plain
 from gpu_util import say
-from test_gpu_mx import TYPES, check_mx, f64, to_dev
+from test_gpu_mx import check_mx, check_product, f64, mx_random, to_dev
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +31,33 @@ def test_norm_past_the_largest_number(fmt, type_, cols, sign):
     y = np.where(np.abs(y) >= 2.0 ** 128 - 2.0 ** 103, np.inf, y)
     assert np.isinf(y).sum() == 1
     check_mx(q, y, fmt)
+
+
+def check_many_rows(rng, act, M, N, seams):
+    """A product with N weight rows of 128 ones, but for 64 random ones at each of `seams`."""
+    free = torch.cuda.mem_get_info()[0]
+    need = N * (64 + 16 + 2 * M) + (8 << 30)
+    if free < need:
+        pytest.skip(f"needs {need >> 30} GiB of device memory")
+    say("many rows", act, M, N)
+    w = vm.MXTensor.empty((N, 128), "fp4")
+    w.codes.fill_(0x22)   # ones
+    w.scales.fill_(127)
+    part, pv = mx_random(rng, (64,), 128, "fp4")
+    for at in seams:
+        w.codes[at:at + 64] = part.codes
+        w.scales[at:at + 64] = part.scales
+    x, xv = mx_random(rng, (M,), 128, act, narrow=True)
+    y = vm.mx_matmul(x, w)
+    check_product(y[:, :1], xv, np.ones((1, 128)), "bf16")
+    for at in seams:
+        check_product(y[:, at:at + 64], xv, pv, "bf16")
+        y[:, at:at + 64] = y[:, :1]
+    for row in y:
+        assert bool((row == row[0]).all())
+
+
+@pytest.mark.parametrize("M,N", [(1, 1 << 30), (17, (1 << 29) + 70)])
+def test_product_many_weight_rows(rng, M, N):
+    """Work-groups of few tokens whose work-items would pass 2^32 in one dimension of a grid."""
+    check_many_rows(rng, "fp8", M, N, [(1 << 27) - 32, (1 << 28) - 32, N - 64])

@@ -18,7 +18,8 @@ k_mx_rows(MxOperand x, MxOperand wt, typename T::Raw* out, long long ldo) {
     __shared__ __attribute__((aligned(256))) unsigned char lds[S::kLds];
     const int lane = lane_id(), n = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const long long row0 = (long long)blockIdx.x * S::R;
+    const long long row0 = group_index() * S::R;
+    if (row0 >= wt.rows) return;  // the whole work-group
     const int rows = (int)min(wt.rows - row0, (long long)S::R), tokens = (int)x.rows;
     S stream;
     stream.init(wt.codes + row0 * mx_code_bytes(x.cols, kMxFp4), wt.scales + row0 * mx_scale_bytes(x.cols),
@@ -54,7 +55,7 @@ k_mx_rows(MxOperand x, MxOperand wt, typename T::Raw* out, long long ldo) {
 
 template <typename T, typename S>
 void launch_rows(const MxOperand& x, const MxOperand& w, void* out, long long ldo, hipStream_t st) {
-    k_mx_rows<T, S><<<(unsigned)((w.rows + S::R - 1) / S::R), 64 * S::W, 0, st>>>(
+    k_mx_rows<T, S><<<grid_of((w.rows + S::R - 1) / S::R), 64 * S::W, 0, st>>>(
         x, w, (typename T::Raw*)out, ldo);
     VCSRMC_HIP(hipGetLastError());
 }
