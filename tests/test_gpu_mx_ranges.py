@@ -35,6 +35,7 @@ def test_norm_past_the_largest_number(fmt, type_, cols, sign):
 
 def check_many_rows(rng, act, M, N, seams):
     """A product with N weight rows of 128 ones, but for 64 random ones at each of `seams`."""
+    torch.cuda.empty_cache()
     free = torch.cuda.mem_get_info()[0]
     need = N * (64 + 16 + 2 * M) + (8 << 30)
     if free < need:
@@ -61,3 +62,10 @@ def check_many_rows(rng, act, M, N, seams):
 def test_product_many_weight_rows(rng, M, N):
     """Work-groups of few tokens whose work-items would pass 2^32 in one dimension of a grid."""
     check_many_rows(rng, "fp8", M, N, [(1 << 27) - 32, (1 << 28) - 32, N - 64])
+
+
+@pytest.mark.parametrize("act", ["fp4", "fp8"])
+@pytest.mark.parametrize("N", [1 << 30, (1 << 29) + 70])
+def test_product_many_tiles(rng, act, N):
+    """2^21 tiles and more, whose work-groups continue in the grid's second dimension."""
+    check_many_rows(rng, act, 33, N, [(1 << 28) - 32, N - 64])

@@ -212,8 +212,10 @@ k_mx_tiles(MxOperand x, MxOperand wt, typename T::Raw* out, long long ldo, unsig
     const int lane = lane_id(), n = lane & 31, b = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n0 = (wave % C::WN) * 32 * C::NT, m0 = (wave / C::WN) * 32 * C::MT;
+    const unsigned id = (unsigned)group_index();
+    if (id >= tn * tm) return;  // the whole work-group
     unsigned bn, bm;
-    tile_of(blockIdx.x, tn * tm, tn, tm, bn, bm);
+    tile_of(id, tn * tm, tn, tm, bn, bm);
     const long long row0 = (long long)bn * C::BN, tok0 = (long long)bm * C::BM;
     const int steps = (int)(mx_padded(x.cols) / kMxStep), quads = (steps + 3) / 4;
     constexpr int kSteps = C::SV / kMxStep;  // of the format's padding, in a stage
@@ -366,8 +368,9 @@ k_mx_tiles(MxOperand x, MxOperand wt, typename T::Raw* out, long long ldo, unsig
 template <typename T, int FX, typename C>
 void launch_tiles(const MxOperand& x, const MxOperand& w, void* out, long long ldo, hipStream_t st) {
     const long long tn = (w.rows + C::BN - 1) / C::BN, tm = (x.rows + C::BM - 1) / C::BM;
-    if (tn * tm >= 1ll << 22) throw Error(VCSRMC_ERR_OVERFLOW, "product too large for one launch");
-    k_mx_tiles<T, FX, C><<<(unsigned)(tn * tm), C::kThreads, 0, st>>>(
+    // more than any memory holds the result of: tiles are counted in 32 bits
+    if (tn * tm >= 1ll << 31) throw Error(VCSRMC_ERR_OVERFLOW, "product too large for one launch");
+    k_mx_tiles<T, FX, C><<<grid_of(tn * tm), C::kThreads, 0, st>>>(
         x, w, (typename T::Raw*)out, ldo, (unsigned)tn, (unsigned)tm);
     VCSRMC_HIP(hipGetLastError());
 }
