@@ -1,5 +1,7 @@
 """What the microscaled operators refuse, before any device work, and their layouts; no GPU."""
 import ctypes
+import pathlib
+import re
 
 import numpy as np
 import pytest
@@ -138,3 +140,15 @@ def test_block_command_refuses(args, capsys):
     with pytest.raises(SystemExit) as e:
         mx_block.main(args)
     assert e.value.code == 2 and "top-k" in capsys.readouterr().err
+
+
+def test_assembly_names_what_it_writes():
+    """Every piece of inline assembly that sets m0 tells the compiler so."""
+    csrc = pathlib.Path(vm.__file__).parent / "csrc"
+    found = 0
+    for path in sorted(csrc.glob("*.h*")):
+        for piece in re.findall(r"\basm\b[^;]*?\((.*?)\);", path.read_text(), re.S):
+            if re.search(r"\bs_mov_b32 m0\b", piece):
+                found += 1
+                assert '"m0"' in piece.rsplit(":", 1)[1], path.name
+    assert found

@@ -217,15 +217,19 @@ __device__ __forceinline__ mx_v8b mx_bf16_of_fp8(unsigned lo, unsigned hi, float
 // copy has no register to wait for, and its reader waits with wait_copies or arrive_but.  It is not
 // the builtin, because the compiler then adds waits of its own before reads of LDS, and with more
 // than a few arrays these wait for every copy on its way.  Waits that it adds for other loads count
-// these copies too, which only makes them longer.  m0 carries the LDS address (one instruction ahead
-// of its use); the compiler keeps nothing in it.
+// these copies too, which only makes them longer.  m0 carries the LDS address, one instruction ahead
+// of its use; it is named as written, so that no use of the compiler's own of m0 is torn apart (the
+// warning is that the compiler would not save a reserved register, of which it never keeps a value).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy16_to_lds(const unsigned char* base, unsigned offset,
                                               unsigned char* to) {
     const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)to;
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset),
                  "s"(base)
-                 : "memory");
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // Where chunks of 16 bytes of a row lie in LDS: chunk c of row r at place c ^ place(r) of its row, so
 // that the 16 lanes that read together (rows 0-3, 12-15, 20-23, 24-27 and the like, or 0-15) touch all
