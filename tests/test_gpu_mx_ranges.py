@@ -69,3 +69,54 @@ def test_product_many_weight_rows(rng, M, N):
 def test_product_many_tiles(rng, act, N):
     """2^21 tiles and more, whose work-groups continue in the grid's second dimension."""
     check_many_rows(rng, act, 33, N, [(1 << 28) - 32, N - 64])
+
+
+def _calls(g):
+    """For every entry point, a call with a stream and the operands that it alone holds."""
+    def normal(*shape):
+        return torch.randn(shape, generator=g, device="cuda")
+
+    w = vm.mx_quantise(normal(512, 1024), "fp4")
+    w13 = vm.mx_quantise(normal(4 * 256, 1024), "fp4")
+    w13 = vm.MXTensor(w13.codes.view(4, 256, -1), w13.scales.view(4, 256, -1), 1024, "fp4")
+    w2 = vm.mx_quantise(normal(4 * 1024, 128), "fp4")
+    w2 = vm.MXTensor(w2.codes.view(4, 1024, -1), w2.scales.view(4, 1024, -1), 128, "fp4")
+    x, r, gain, router = normal(96, 1024), normal(96, 1024), normal(1024), normal(4, 1024)
+    q = vm.mx_quantise(x)
+    return {"quantise": (lambda x, s: vm.mx_quantise(x, stream=s).codes, [x]),
+            "dequantise": (lambda c, e, s: vm.mx_dequantise(vm.MXTensor(c, e, 1024, "fp8"), stream=s),
+                           [q.codes, q.scales]),
+            "norm": (lambda x, r, w, s: vm.rms_norm_mx(x, w, residual=r, stream=s)[1], [x, r, gain]),
+            "matmul": (lambda c, e, s: vm.mx_matmul(vm.MXTensor(c, e, 1024, "fp8"), w, stream=s),
+                       [q.codes, q.scales]),
+            "moe": (lambda c, e, r, s: vm.mx_moe(vm.MXTensor(c, e, 1024, "fp8"), r, w13, w2, 2, stream=s),
+                    [q.codes, q.scales, router])}
+
+
+@pytest.mark.parametrize("name", ["quantise", "dequantise", "norm", "matmul", "moe"])
+def test_operands_dropped_before_their_stream_is_done(name):
+    """What the caller drops behind a call on another stream keeps its memory until that stream has
+    passed the call, and the result is right."""
+    say("dropped operands", name)
+    call, held = _calls(torch.Generator(device="cuda").manual_seed(3))[name]
+    want = call(*held, None)
+    side, busy = torch.cuda.Stream(), torch.randn((8192, 8192), device="cuda")
+    out = torch.empty_like(busy)
+    torch.matmul(busy, busy, out=out)
+    operands = [t.clone() for t in held]
+    where = {t.data_ptr() for t in operands}
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(30):
+            torch.matmul(busy, busy, out=out)
+    got = call(*operands, side)
+    sizes = [t.numel() * t.element_size() for t in operands]
+    del operands
+    new = [torch.empty((n,), dtype=torch.uint8, device="cuda") for n in sizes for _ in range(4)]
+    late = not side.query()
+    taken = where & {t.data_ptr() for t in new}
+    for t in new:
+        t.fill_(0xff)
+    side.synchronize()
+    assert late and not taken
+    assert torch.equal(got, want)

@@ -6,6 +6,11 @@ their product with the weights (``mx_matmul``) and a whole mixture-of-experts la
 tokens (``mx_moe``).  Thin wrappers of the C ABI (include/vcsrmc.h, "microscaled operators"): they
 check their operands on the host, allocate what the caller does not give, and launch on ``stream``
 (default: torch's current stream of the operands' device) without waiting.
+
+``stream`` is a torch stream or the handle of any other.  Operands are to be ready on it (the caller
+lets it wait for the streams that make them).  A caller may drop them at once where it is a torch
+stream: their memory is kept for it.  Under the handle of another stream, or an ExternalStream of
+it, the caller keeps them until the call has run.
 """
 from __future__ import annotations
 
@@ -117,14 +122,23 @@ class MXTensor:
 
 
 @contextlib.contextmanager
-def _on(device, stream):
-    """`device` and `stream` current: what is allocated inside belongs to that stream.  The entry
-    points enter it only where they are not current already: it costs more than a small launch."""
+def _on(device, stream, *operands):
+    """`device` and `stream` current: what is allocated inside belongs to that stream, and what the
+    caller frees of the operands is not used again before that stream has passed the call.  The
+    entry points enter it only where they are not current already: it costs more than a small
+    launch."""
     with torch.cuda.device(device):
+        given = stream
         if isinstance(stream, int):
             stream = torch.cuda.ExternalStream(stream, device=device)
         with torch.cuda.stream(stream):
             yield
+        # a stream that is not torch's may be gone when the operand is freed: its owner keeps them
+        if isinstance(given, torch.cuda.Stream) and not isinstance(given, torch.cuda.ExternalStream):
+            for t in operands:
+                for part in (t.codes, t.scales) if isinstance(t, MXTensor) else (t,):
+                    if part is not None:
+                        part.record_stream(given)
 
 
 def _matrix(t, name: str, rows: int | None = None, cols: int | None = None, like=None):
@@ -180,7 +194,7 @@ def mx_quantise(x, fmt: str = "fp8", out: MXTensor | None = None, stream=None) -
     ld = _matrix(x, "x")
     at = x.get_device()
     if stream is not None or at != _current_device():
-        with _on(x.device, stream):
+        with _on(x.device, stream, x, out):
             return mx_quantise(x, fmt, out)
     rows, cols = x.shape
     q = _mx_out(out, rows, cols, fmt, x)
@@ -196,7 +210,7 @@ def mx_dequantise(q: MXTensor, dtype=torch.float32, out=None, stream=None):
     _mx(q, "q")
     at = q.codes.get_device()
     if stream is not None or at != _current_device():
-        with _on(q.device, stream):
+        with _on(q.device, stream, q, out):
             return mx_dequantise(q, dtype, out)
     o, ld = _plain_out(out, q.rows, q.cols, dtype, q.codes)
     rc = lib().vcsrmc_mx_dequantise(q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.cols, q.bits,
@@ -230,7 +244,7 @@ def rms_norm_mx(x, weight, residual=None, eps: float = 1e-6, fmt: str = "fp8",
     elif residual_out is not None:
         _refuse("residual_out needs a residual")
     if stream is not None or at != _current_device():
-        with _on(x.device, stream):
+        with _on(x.device, stream, x, weight, residual, out, residual_out):
             return rms_norm_mx(x, weight, residual, eps, fmt, out, residual_out)
     q = _mx_out(out, rows, cols, fmt, x)
     h = residual_out
@@ -262,7 +276,7 @@ def mx_matmul(x: MXTensor, w: MXTensor, dtype=torch.bfloat16, out=None, stream=N
     if K != w.cols or at != wc.get_device():
         _refuse(f"x has rows of {K} values on {x.device}, w of {w.cols} on {w.device}")
     if stream is not None or at != _current_device():
-        with _on(x.device, stream):
+        with _on(x.device, stream, x, w, out):
             return mx_matmul(x, w, dtype, out)
     if N == 0:
         return xc.new_empty((M, 0), dtype=dtype)
@@ -299,7 +313,7 @@ def mx_moe(x: MXTensor, router, w13: MXTensor, w2: MXTensor, top_k: int, renorma
         _refuse(f"experts must be 1 to {MAX_EXPERTS} and top_k 1 to experts (at most {MAX_TOP_K}), "
                 f"not {E} and {top_k}")
     if stream is not None or at != _current_device():
-        with _on(x.device, stream):
+        with _on(x.device, stream, x, router, w13, w2, out):
             return mx_moe(x, router, w13, w2, top_k, renormalise, dtype, out)
     o, ld = _plain_out(out, T, D, dtype, xc)
     need = _moe_workspace(T, D, F, E, top_k)
