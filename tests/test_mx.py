@@ -2,6 +2,7 @@
 import ctypes
 import pathlib
 import re
+import types
 
 import numpy as np
 import pytest
@@ -60,6 +61,17 @@ def test_tensors_must_be_on_the_device():
     refused(lambda: vm.mx_matmul(x, x), "MXTensor")
     refused(lambda: vm.mx_moe(x, x, x, x, 1), "MXTensor")
     refused(lambda: vm.mx_dequantise(x), "MXTensor")
+
+
+def test_streams_of_another_device():
+    """Refused, not passed over for that device's current stream."""
+    other = types.SimpleNamespace(device=torch.device("cuda:1"))
+
+    def enter():
+        with mx._on(torch.device("cuda:0"), other):
+            pass
+
+    refused(enter, "stream", "cuda:1", "cuda:0")
 
 
 A = 4096  # an address that is never read: every call below is refused first

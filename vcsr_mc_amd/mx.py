@@ -127,6 +127,8 @@ def _on(device, stream, *operands):
     caller frees of the operands is not used again before that stream has passed the call.  The
     entry points enter it only where they are not current already: it costs more than a small
     launch."""
+    if getattr(stream, "device", device) != device:
+        _refuse(f"the stream is of {stream.device}, the operands are on {device}")
     with torch.cuda.device(device):
         given = stream
         if isinstance(stream, int):
