@@ -120,3 +120,25 @@ def test_operands_dropped_before_their_stream_is_done(name):
     side.synchronize()
     assert late and not taken
     assert torch.equal(got, want)
+
+
+def test_gradients_are_refused_not_lost():
+    """The sum that a norm returns and a layer's output carry no gradient: who asks for one is told."""
+    say("gradients")
+    calls = _calls(torch.Generator(device="cuda").manual_seed(3))
+    norm, (x, r, gain) = calls["norm"]
+    moe, (codes, scales, router) = calls["moe"]
+    want_h, want_y = norm(x, r, gain, None), moe(codes, scales, router, None)
+    asks = [t.clone().requires_grad_() for t in (x, r, router)]
+    for call in (lambda: norm(asks[0], r, gain, None), lambda: norm(x, asks[1], gain, None),
+                 lambda: moe(codes, scales, asks[2], None)):
+        with pytest.raises(vm.VCSRMCError, match="no_grad") as e:
+            call()
+        assert e.value.status == vm.ERR_ARG
+    # in codes nothing is lost that torch could follow; a weight does not reach the sum
+    assert torch.equal(vm.rms_norm_mx(asks[0], gain)[0].codes, vm.rms_norm_mx(x, gain)[0].codes)
+    assert torch.equal(norm(x, r, torch.nn.Parameter(gain), None), want_h)
+    assert torch.equal(vm.mx_quantise(asks[0]).codes, vm.mx_quantise(x).codes)
+    with torch.no_grad():
+        assert torch.equal(norm(asks[0], asks[1], gain, None), want_h)
+        assert torch.equal(moe(codes, scales, asks[2], None), want_y)

@@ -11,6 +11,9 @@ check their operands on the host, allocate what the caller does not give, and la
 lets it wait for the streams that make them).  A caller may drop them at once where it is a torch
 stream: their memory is kept for it.  Under the handle of another stream, or an ExternalStream of
 it, the caller keeps them until the call has run.
+
+For serving: nothing here has a gradient.  Where a result in 16 or 32 bits would lose one silently,
+the operand that requires it is refused, as long as torch records gradients.
 """
 from __future__ import annotations
 
@@ -32,6 +35,12 @@ _U8 = torch.uint8
 
 def _refuse(msg: str):
     raise VCSRMCError(ERR_ARG, msg)
+
+
+def _no_gradient(what: str, *operands):
+    """Refuses operands whose gradient a result would have to carry: none of these has one."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
+        _refuse(f"{what} has no gradient: call under torch.no_grad(), or detach what requires one")
 
 
 def _format(fmt) -> int:
@@ -226,7 +235,8 @@ def rms_norm_mx(x, weight, residual=None, eps: float = 1e-6, fmt: str = "fp8",
                 out: MXTensor | None = None, residual_out=None, stream=None):
     """(MX of h / sqrt(mean(h^2) + eps) * weight, h) with h = x + residual, row by row in 32 bits;
     the second is h rounded to x's type, None without a residual.  residual_out may be x or
-    residual themselves."""
+    residual themselves.  h carries no gradient: under a residual, x and residual that require one
+    are refused."""
     bits = _format(fmt)
     ldx = _matrix(x, "x")
     rows, cols = x.shape
@@ -239,6 +249,7 @@ def rms_norm_mx(x, weight, residual=None, eps: float = 1e-6, fmt: str = "fp8",
         ldr = _matrix(residual, "residual", rows, cols, x)
         if residual.dtype is not dtype:
             _refuse("residual must have x's type")
+        _no_gradient("rms_norm_mx's sum", x, residual)
         if residual_out is not None:
             ldo = _matrix(residual_out, "residual_out", rows, cols, x)
             if residual_out.dtype is not dtype:
@@ -296,7 +307,8 @@ def mx_moe(x: MXTensor, router, w13: MXTensor, w2: MXTensor, top_k: int, renorma
     """A mixture-of-experts layer: x (T x D, fp8), router (E x D), w13 (E x 2F x D, fp4: F gate
     rows, then F up rows) and w2 (E x D x F, fp4).  Each token's top_k experts by router . x (ties
     to the lower index), weighted by softmax over them (renormalise) or over all experts.  For
-    decoding batches: tokens are taken 64 at a time, each time with the weights of their experts."""
+    decoding batches: tokens are taken 64 at a time, each time with the weights of their experts.
+    No gradient: a router that requires one is refused."""
     _mx(x, "x", "fp8")
     _mx(w13, "w13", "fp4")
     _mx(w2, "w2", "fp4")
@@ -311,6 +323,7 @@ def mx_moe(x: MXTensor, router, w13: MXTensor, w2: MXTensor, top_k: int, renorma
     at = xc.get_device()
     if not at == router.get_device() == w13c.get_device() == w2c.get_device():
         _refuse("x, router, w13 and w2 must be on the same GPU")
+    _no_gradient("mx_moe", router)
     if not 1 <= E <= MAX_EXPERTS or not 1 <= top_k <= min(E, MAX_TOP_K):
         _refuse(f"experts must be 1 to {MAX_EXPERTS} and top_k 1 to experts (at most {MAX_TOP_K}), "
                 f"not {E} and {top_k}")
