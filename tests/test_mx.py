@@ -1,5 +1,6 @@
 """What the microscaled operators refuse, before any device work, and their layouts; no GPU."""
 import ctypes
+import importlib.util
 import pathlib
 import re
 import types
@@ -61,6 +62,19 @@ def test_tensors_must_be_on_the_device():
     refused(lambda: vm.mx_matmul(x, x), "MXTensor")
     refused(lambda: vm.mx_moe(x, x, x, x, 1), "MXTensor")
     refused(lambda: vm.mx_dequantise(x), "MXTensor")
+
+
+def test_torch_without_its_private_names(monkeypatch):
+    """The module loads, and finds devices and streams by torch's public functions."""
+    for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+        monkeypatch.delattr(torch._C, name, raising=False)
+    spec = importlib.util.spec_from_file_location("vcsr_mc_amd.mx_again", mx.__file__)
+    again = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(again)
+    assert again._current_device is torch.cuda.current_device
+    monkeypatch.setattr(torch.cuda, "current_stream",
+                        lambda device: types.SimpleNamespace(cuda_stream=70 + device))
+    assert again._current_stream(2) == 72
 
 
 def test_streams_of_another_device():

@@ -28,8 +28,11 @@ from . import ERR_ARG, VCSRMCError, _check, lib
 FORMATS = {"fp4": 4, "fp8": 8}
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 MAX_EXPERTS, MAX_TOP_K = 1024, 64
-_current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
+# Without the checks and the objects of torch's public functions, which cost more than a small
+# launch does; those serve where a torch lacks these.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                          lambda device: torch.cuda.current_stream(device).cuda_stream)
 _U8 = torch.uint8
 
 
