@@ -325,6 +325,9 @@ int vcsrmc_mx_matmul(const void *x_codes, const void *x_scales, int x_format, lo
  * experts by l (equal ones: the lower index first; NaN last) under p = softmax of l over the
  * chosen (renormalise = 1) or over all experts (0); h = silu(gate x) * (up x), rounded to
  * VCSRMC_MX_FP8 for the second product; out (T x D of `type`, row stride ldo) = sum of p (w2 h).
+ * Logits, gate and up sums take values in 32-bit range: x's scales up to 246 and w13's up to 252 (the
+ * most that quantisation writes), and of x under scales 0 to 2 what lies below 2^-133 may be lost.
+ * The second product cuts as vcsrmc_mx_matmul's does with VCSRMC_MX_FP8.
  * E is at most 1024, top_k at most 64, D and F at most 2^22, and the codes of an expert's w13 at
  * most 2^32 bytes.  Tokens are taken 64 at a time: the weights of chosen experts are read anew for
  * each 64, and for each 16, 32 or 64 of them that share an expert.  Deterministic. */

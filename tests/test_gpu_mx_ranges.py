@@ -4,7 +4,8 @@ import pytest
 
 import mx_plain as plain
 from gpu_util import say
-from test_gpu_mx import check_mx, check_product, f64, mx_random, to_dev
+from test_gpu_mx import (ACTS, TAU, act_of, check_moe, check_mx, check_product, f64, moe_case, mx_random,
+                         to_dev)
 
 pytestmark = pytest.mark.gpu
 
@@ -13,6 +14,7 @@ torch = pytest.importorskip("torch")
 import vcsr_mc_amd as vm  # noqa: E402
 
 
+# ---- values ----------------------------------------------------------------------------------
 @pytest.mark.parametrize("fmt", ["fp8", "fp4"])
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
 @pytest.mark.parametrize("cols", [96, 5000, 40000])
@@ -33,6 +35,44 @@ def test_norm_past_the_largest_number(fmt, type_, cols, sign):
     check_mx(q, y, fmt)
 
 
+# ---- scales ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("act,narrow", [("fp8", True), ("fp4", False)])
+@pytest.mark.parametrize("mid_x,mid_w", [(2, 250), (5, 248), (250, 4), (252, 2)])
+@pytest.mark.parametrize("M", [1, 20, 100])
+def test_product_scales(rng, act, narrow, mid_x, mid_w, M):
+    """Scales of X at one end of their range, of W at the other: products are of normal size."""
+    say("product scales", act, mid_x, mid_w, M)
+    x, xv = mx_random(rng, (M,), 300, act, mid=mid_x, narrow=narrow)
+    w, wv = mx_random(rng, (200,), 300, "fp4", mid=mid_w)
+    check_product(vm.mx_matmul(x, w, dtype=torch.float32), xv, wv, "f32")
+
+
+@pytest.mark.parametrize("mid_x,mid_w", [(5, 235), (9, 231), (60, 180), (244, 8)])
+@pytest.mark.parametrize("T,D,F,E", [(1, 256, 64, 2), (3, 200, 100, 2), (20, 300, 64, 3)])
+def test_moe_scales(rng, mid_x, mid_w, T, D, F, E):
+    """Scales of x and of the gate and up rows far apart, bytes 3 to 246: h is of normal size."""
+    say("moe scales", mid_x, mid_w, T, D, F, E)
+    x, xv = mx_random(rng, (T,), D, "fp8", mid=mid_x)
+    w13, a = mx_random(rng, (E, 2 * F), D, "fp4", mid=mid_w)
+    w2, b = mx_random(rng, (E, D), F, "fp4", mid=119)
+    y = vm.mx_moe(x, torch.zeros((E, D), device="cuda"), w13, w2, E, dtype=torch.float32)
+    with np.errstate(over="ignore"):  # sigmoid of large gates
+        check_moe(y, (xv, np.zeros((E, D)), a, b), E, True, "f32", router_gap=False)
+
+
+@pytest.mark.parametrize("T", [1, 3, 20])
+def test_moe_router_of_tiny_activations(rng, T):
+    """Activations below 2^-126 under a large router: logits of normal size choose as they should."""
+    D, F, E, k = 256, 64, 8, 2
+    x, xv = mx_random(rng, (T,), D, "fp8", mid=5, narrow=True)
+    router = to_dev(rng.standard_normal((E, D)) * 2.0 ** 118)
+    w13, a = mx_random(rng, (E, 2 * F), D, "fp4", mid=233)
+    w2, b = mx_random(rng, (E, D), F, "fp4", mid=119)
+    y = vm.mx_moe(x, router, w13, w2, k, dtype=torch.float32)
+    check_moe(y, (xv, f64(router), a, b), k, True, "f32")
+
+
+# ---- sizes -----------------------------------------------------------------------------------
 def check_many_rows(rng, act, M, N, seams):
     """A product with N weight rows of 128 ones, but for 64 random ones at each of `seams`."""
     torch.cuda.empty_cache()
@@ -71,6 +111,7 @@ def test_product_many_tiles(rng, act, N):
     check_many_rows(rng, act, 33, N, [(1 << 28) - 32, N - 64])
 
 
+# ---- streams and gradients -------------------------------------------------------------------
 def _calls(g):
     """For every entry point, a call with a stream and the operands that it alone holds."""
     def normal(*shape):

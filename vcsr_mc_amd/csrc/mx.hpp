@@ -181,9 +181,11 @@ __device__ __forceinline__ unsigned word_of(const uint4& v, int i) {
 template <int FX> constexpr int kMxStepBytes = FX == kMxFp8 ? 128 : 64;
 
 // ---- matrix steps with nothing lost -----------------------------------------------------------
-// The same products through bfloat16, which holds every value of FP8 and FP4 under its scale, on
-// v_mfma_f32_16x16x32_bf16: products exact, sums in 32 bits, where the FP8 path cuts the smaller
-// products of 8 neighbours (2^-13 of the largest).  For sums that are rounded to 8 bits again:
+// The same products through bfloat16 on v_mfma_f32_16x16x32_bf16: products exact, sums in 32 bits,
+// where the FP8 path cuts the smaller products of 8 neighbours (2^-13 of the largest).  bfloat16 holds
+// every value of FP8 under scale bytes 3 to 246 and of FP4 under 0 to 252; quantisation writes none
+// above these.  Under 0 to 2 FP8 values lose what lies below 2^-133 (the least are 2^-136); above 246
+// and 252 values past 2^128 become infinities, where the scaled instructions go on.  For sums that are rounded to 8 bits again:
 // there the cut moves values across rounding boundaries, a step of 2^-4 each.  The conversions
 // cost 16 vector instructions per operand and step, hidden where the weights come from memory.
 // Lane (n, q) holds block q of the step on both sides; instruction j takes its values 8 j .. + 7.
