@@ -4,7 +4,7 @@ import pytest
 
 import mx_plain as plain
 from gpu_util import say
-from test_gpu_mx import (ACTS, TAU, act_of, check_moe, check_mx, check_product, f64, moe_case, mx_random,
+from test_gpu_mx import (ACTS, act_of, check_moe, check_mx, check_product, f64, moe_case, mx_random,
                          to_dev)
 
 pytestmark = pytest.mark.gpu
@@ -33,6 +33,51 @@ def test_norm_past_the_largest_number(fmt, type_, cols, sign):
     y = np.where(np.abs(y) >= 2.0 ** 128 - 2.0 ** 103, np.inf, y)
     assert np.isinf(y).sum() == 1
     check_mx(q, y, fmt)
+
+
+def check_norm_exact(q, x, r, w, eps):
+    """Scales and codes are those of the normalised values in 64 bits, rounded once.  Those values
+    carry a few roundings of 2^-53 on either side, so where a change by 1e-12 of them changes a code
+    or a scale, either is right; such places are a few in a million at most."""
+    h = x.float() if r is None else x.float() + r.float()   # the norm's h has 32 bits
+    y, _ = plain.norm(f64(h), None, f64(w), np.float32(eps))
+    cols = y.shape[1]
+    nb = plain.pad(cols, 32) // 32
+    got_c, got_s = q.codes.cpu().numpy(), q.scales.cpu().numpy()
+    right_v, right_s, values, scales = 0, 0, [], []
+    got = plain.unpack(got_c, got_s, cols, q.fmt)
+    for f in (1, 1 - 1e-12, 1 + 1e-12):
+        c, s = plain.quantise(y * f, q.fmt)
+        values.append(plain.values(c, s, q.fmt)[:, :cols])
+        scales.append(s)
+        right_v |= got == values[-1]
+        right_s |= got_s[:, :nb] == s
+    assert np.all(right_s) and np.all(right_v)
+    assert np.mean(values[1] != values[2]) <= 1e-5 + 1 / y.size
+    assert np.mean(scales[1] != scales[2]) <= 1e-5 + 1 / scales[0].size
+    assert not np.any(got_s[:, nb:])
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("type_,wtype", [("f32", "f32"), ("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"),
+                                         ("bf16", "f32")])
+@pytest.mark.parametrize("rows,cols,residual", [(1, 1, True), (3, 100, False), (2, 511, True), (40, 4096, True),
+                                                (33, 5000, False), (20, 8200, True), (9, 33000, True)])
+def test_norm_rounds_once(rng, fmt, type_, wtype, rows, cols, residual):
+    say("norm exact", fmt, type_, wtype, rows, cols, residual)
+    x = to_dev(rng.standard_normal((rows, cols)) * 3, type_)
+    r = to_dev(rng.standard_normal((rows, cols)), type_) if residual else None
+    w = to_dev(1 + 0.2 * rng.standard_normal(cols), wtype)
+    q, _ = vm.rms_norm_mx(x, w, residual=r, eps=1e-5, fmt=fmt)
+    check_norm_exact(q, x, r, w, 1e-5)
+
+
+def test_norm_rounds_once_over_many(rng):
+    """17 million values: what a norm in 32 bits gets wrong a few times in a million."""
+    x, r = (to_dev(rng.standard_normal((2100, 8192), np.float32)) for _ in range(2))
+    w = to_dev(1 + 0.2 * rng.standard_normal(8192))
+    q, _ = vm.rms_norm_mx(x, w, residual=r, eps=1e-5)
+    check_norm_exact(q, x, r, w, 1e-5)
 
 
 # ---- scales ----------------------------------------------------------------------------------
@@ -72,6 +117,89 @@ def test_moe_router_of_tiny_activations(rng, T):
     check_moe(y, (xv, f64(router), a, b), k, True, "f32")
 
 
+# ---- experts -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("T", [1, 5, 40])
+@pytest.mark.parametrize("D,router_type", [(1024, "f32"), (1025, "f32"), (2049, "bf16"), (2500, "f32"), (3100, "f16"),
+                                           (4000, "bf16"), (4224, "f32"), (9000, "f32")])
+def test_moe_logits_in_parts(rng, T, D, router_type):
+    """Routers' rows in one to four parts."""
+    say("moe parts", T, D, router_type)
+    ops, v = moe_case(rng, T, D, 64, 20, router_type)
+    check_moe(vm.mx_moe(*ops, 3, renormalise=False, dtype=torch.float32), v, 3, False, "f32")
+
+
+@pytest.mark.parametrize("T", [1, 6, 40])
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+@pytest.mark.parametrize("E,k", [(6, 2), (100, 3)])
+def test_moe_infinite_logits(rng, T, value, E, k):
+    """An infinite logit of one or of all experts.  A softmax over +inf is NaN; -inf comes after all
+    finite ones and has weight zero where it is chosen."""
+    say("moe infinite", T, value, E, k)
+    (x, router, w13, w2), v = moe_case(rng, T, 96, 32, E)
+    x.codes[:, 7] = 0x38     # the value whose weight in the router is infinite is positive
+    xv = plain.unpack(x.codes.cpu().numpy(), x.scales.cpu().numpy(), 96, "fp8")
+    one = router.clone()
+    one[E - 1, 7] = value
+    y = vm.mx_moe(x, one, w13, w2, k, dtype=torch.float32)
+    if value > 0:
+        assert torch.all(torch.isnan(y))
+    else:  # as if that expert were the least of all
+        r = f64(router)
+        ids = plain.choose(np.where(np.arange(E) == E - 1, -np.inf, xv @ r.T), k)
+        assert not np.any(ids == E - 1)
+        check_moe(y, (xv, r[:E - 1], v[2][:E - 1], v[3][:E - 1]), k, True, "f32")
+    router[:, 7] = value
+    assert torch.all(torch.isnan(vm.mx_moe(x, router, w13, w2, k, dtype=torch.float32)))
+
+
+def test_moe_chosen_at_minus_infinity(rng):
+    """All experts are chosen, one of them at -inf: it has weight zero."""
+    (x, router, w13, w2), (xv, r, a, b) = moe_case(rng, 5, 96, 32, 4)
+    x.codes[:, 7] = 0x38
+    xv = plain.unpack(x.codes.cpu().numpy(), x.scales.cpu().numpy(), 96, "fp8")
+    router[2, 7] = -np.inf
+    rest = [0, 1, 3]
+    for renormalise in (True, False):
+        y = vm.mx_moe(x, router, w13, w2, 4, renormalise=renormalise, dtype=torch.float32)
+        check_moe(y, (xv, r[rest], a[rest], b[rest]), 3, renormalise, "f32")
+
+
+class Experts:
+    """float64 values of an MX tensor's matrices, made when they are asked for."""
+
+    def __init__(self, q):
+        self.q, self.shape, self.made = q, q.shape, {}
+        byte = np.arange(256)
+        pairs = np.stack((byte & 15, byte >> 4), -1)
+        self.pairs = np.where(pairs >= 8, -1, 1) * plain.GRID["fp4"][pairs % 8]
+
+    def __getitem__(self, e):
+        if e not in self.made:
+            v = self.pairs[self.q.codes[int(e)].cpu().numpy()].reshape(self.shape[1], -1, 32)
+            s = np.ldexp(1.0, self.q.scales[int(e)].cpu().numpy().astype(int) - 127)
+            self.made[e] = (v * s[:, :v.shape[1], None]).reshape(self.shape[1], -1)[:, :self.shape[2]]
+        return self.made[e]
+
+
+@pytest.mark.parametrize("T,k,rows", [(1, 4, [0]), (1, 8, [0]), (7, 6, [0, 6]), (64, 8, [0, 31, 63])])
+def test_moe_full_layer(rng, T, k, rows):
+    """64 experts of 4096 x 2048: some tokens' results against the definition."""
+    D, F, E = 4096, 2048, 64
+    say("moe full", T, k)
+    g = torch.Generator(device="cuda").manual_seed(T)
+
+    def weights(n, cols):
+        codes = torch.randint(0, 256, (E, n, cols // 2), dtype=torch.uint8, device="cuda", generator=g)
+        return vm.MXTensor(codes, torch.randint(117, 121, (E, n, cols // 32), dtype=torch.uint8, device="cuda",
+                                                generator=g), cols, "fp4")
+
+    w13, w2 = weights(2 * F, D), weights(D, F)
+    x, xv = mx_random(rng, (T,), D, "fp8", mid=121, narrow=True)
+    router = to_dev(rng.standard_normal((E, D)) / np.sqrt(D) / 4, "bf16")
+    y = vm.mx_moe(x, router, w13, w2, k, dtype=torch.float32)
+    check_moe(y[rows], (xv[rows], f64(router), Experts(w13), Experts(w2)), k, True, "f32")
+
+
 # ---- sizes -----------------------------------------------------------------------------------
 def check_many_rows(rng, act, M, N, seams):
     """A product with N weight rows of 128 ones, but for 64 random ones at each of `seams`."""
@@ -96,6 +224,8 @@ def check_many_rows(rng, act, M, N, seams):
         y[:, at:at + 64] = y[:, :1]
     for row in y:
         assert bool((row == row[0]).all())
+    del w, y, row
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("M,N", [(1, 1 << 30), (17, (1 << 29) + 70)])
@@ -109,6 +239,36 @@ def test_product_many_weight_rows(rng, M, N):
 def test_product_many_tiles(rng, act, N):
     """2^21 tiles and more, whose work-groups continue in the grid's second dimension."""
     check_many_rows(rng, act, 33, N, [(1 << 28) - 32, N - 64])
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M,N,K", [(33, 50000, 200), (64, 50000, 130), (65, 50000, 400), (33, 25000, 1030)])
+def test_product_few_tokens_many_rows(rng, act, M, N, K):
+    """The largest tiles, mostly empty along the tokens."""
+    say("product wide", act, M, N, K)
+    x, xv, tau = act_of(rng, M, K, act)
+    w, wv = mx_random(rng, (N,), K, "fp4")
+    check_product(vm.mx_matmul(x, w, dtype=torch.float32), xv, wv, "f32", tau)
+
+
+@pytest.mark.parametrize("act", ["fp8", "fp4"])
+def test_product_tiles_far_offsets(rng, act):
+    """Tiles of weights and of results past 4 GB: rows of ones, and random ones at the end."""
+    M, N, K = 2100, 1_100_000, 8192
+    say("product tiles far", act)
+    w = vm.MXTensor.empty((N, K), "fp4")
+    w.codes.fill_(0x22)   # ones
+    w.scales.fill_(127)
+    part, pv = mx_random(rng, (64,), K, "fp4")
+    w.codes[-64:] = part.codes
+    w.scales[-64:] = part.scales
+    x, xv = mx_random(rng, (M,), K, act, narrow=True)
+    y = vm.mx_matmul(x, w)
+    assert w.codes.numel() > 1 << 32 and y.numel() * 2 > 1 << 32
+    check_product(y[:, -64:], xv, pv, "bf16")
+    check_product(y[:, :1], xv, np.ones((1, K)), "bf16")
+    for t in range(0, M, 100):
+        assert bool((y[t:t + 100, :-64] == y[t:t + 100, :1]).all())
 
 
 # ---- streams and gradients -------------------------------------------------------------------
