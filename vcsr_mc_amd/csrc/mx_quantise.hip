@@ -130,8 +130,9 @@ __device__ __forceinline__ void load_h(const RmsNormArgs& a, long long row, int 
 __device__ __forceinline__ float round_to_odd(double v) {
     const float f = (float)v;
     const double d = v - (double)f;  // not finite where f is not
+    constexpr int kFiniteNonzero = 0x198;  // classes: normal and subnormal numbers of either sign
     const unsigned u = __float_as_uint(f);
-    if ((u & 1) || !(fabs(d) > 0 && fabs(d) < HUGE_VAL)) return f;
+    if ((u & 1) || !__builtin_amdgcn_class(d, kFiniteNonzero)) return f;
     return __uint_as_float((d > 0) == !(u >> 31) ? u + 1 : u - 1);
 }
 
