@@ -4,8 +4,8 @@
 // A lane holds 8 consecutive values (one 16-byte load of a 16-bit type), so 4 lanes hold a block:
 // its largest magnitude is two DPP steps away, and no value passes through LDS.  All kernels here
 // are one pass over their data, bound by HBM: 8192 x 8192 bfloat16 to FP4 (170 MB) in 36 us, 4.7 TB/s;
-// the norm of 16384 x 8192 with residual (943 MB) in 193 us, 4.9 TB/s.  A copy of such size reaches 4.7
-// to 5.3.
+// the norm of 16384 x 8192 with residual (943 MB) in 195 us a call among others, 4.8 TB/s (traced
+// alone 198 to 210).  A copy of such size reaches 4.7 to 5.3.
 #include "internal.hpp"
 #include "mx.hpp"
 
@@ -218,8 +218,8 @@ void launch_norm(const RmsNormArgs& a, hipStream_t st) {
     const bool wvec = aligned16(a.weight, 0, sizeof(typename W::Raw));
     const dim3 grid = grid_of(a.rows);
     const long long units = mx_scale_bytes(a.cols) * 4;  // a multiple of 64
-    // Units a thread: 16384 rows of 8192 bfloat16 take 205 us with 2, 238 with 1 (fewer rows on a CU
-    // at once) and 232 with 4; 256 rows 7.1, 7.2 and 9.0 us.
+    // Units a thread, kernels traced alone: 16384 rows of 8192 bfloat16 take 205 us with 2, 238 with 1
+    // (fewer rows on a CU at once) and 232 with 4; 256 rows 7.1, 7.2 and 9.0 us.
     auto threads = [&](int v) { return (int)((units / v + 63) / 64 * 64); };
     if (units < 512) k_rms_norm_mx<T, W, 1><<<grid, threads(1), 0, st>>>(a, vec, wvec);
     else if (units <= 2048) k_rms_norm_mx<T, W, 2><<<grid, threads(2), 0, st>>>(a, vec, wvec);
